@@ -1,0 +1,53 @@
+"""What a step of drafted trees leaves in a decode state, and what it takes from its arguments."""
+import numpy as np
+import pytest
+import torch
+
+from tests.test_drafted_gpu import DEV, SPECS, _close, _model, _prefilled
+from ultraviolet_b200.drafted import TreeRunner, generate_drafted
+
+pytestmark = pytest.mark.gpu
+
+
+def _caches(st, rows=slice(None)):
+    return [t[rows].clone() for y in (st.k, st.v, st.k_scale, st.v_scale) for t in y]
+
+
+def _same(a, b):
+    return all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def _runner(m, prompts, max_new, slots=0, **kw):
+    """A runner over the prompts (of one length), prefilled."""
+    text = torch.tensor(prompts)
+    B, n = text.shape
+    st = m.new_state(B, slots or n + max_new + 2 * 64)
+    if n > 1:
+        m.prefill(text[:, :-1].to(DEV), torch.zeros(B, dtype=torch.long, device=DEV), st)
+    return TreeRunner(m, st, text.int().to(DEV), torch.full((B,), n), max_new, **kw)
+
+
+def _favour(m, *tokens):
+    """Biases that make every draw one of the tokens, the first one first."""
+    return dict(bias_ids=torch.tensor(tokens, dtype=torch.int32, device=DEV),
+                bias=torch.tensor([1e4 - 100 * i for i in range(len(tokens))], device=DEV))
+
+
+@pytest.mark.parametrize("name", sorted(SPECS))
+def test_capturing_a_step_leaves_the_state_as_it_is(name):
+    """Prompts longer than the window, so that an accepted path wraps over ring slots that the first step still reads, and a first draft
+    that is accepted for certain: the text ends in a token that every draw is."""
+    m = _model(name)
+    V, n = m.cfg.vocab_size, m.cfg.window + 9
+    r = np.random.default_rng(3)
+    prompts = [r.integers(20, V, n - 4).tolist() + [7] * 4 for _ in range(3)]
+    runs = [_runner(m, prompts, 20, branches=1, depth=5, temperature=0.0, seed=1, use_graph=g, **_favour(m, 7)) for g in (True, False)]
+    graph, eager = runs
+    before, pos = _caches(graph.st), graph.st.pos.clone()
+    graph._capture()
+    assert _same(_caches(graph.st), before) and torch.equal(graph.st.pos, pos) and int(graph.drawn.max()) == 0
+    for run in runs:
+        run.step()
+        assert run.drawn.tolist() == [6] * 3 and torch.equal(run.st.pos, pos + 6)
+    _close(graph.logits, eager.logits)
+    m.engine.check_status()

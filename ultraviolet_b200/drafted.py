@@ -138,7 +138,9 @@ class TreeRunner:
         saved = [t.clone() for t in kept]
         s = torch.cuda.Stream(dev)
         s.wait_stream(torch.cuda.current_stream(dev))
-        with torch.cuda.stream(s):  # warm-up: what it writes to the caches is rewritten by the real replay
+        with torch.cuda.stream(s):
+            # warm-up without a node in any tree: an accepted path would wrap over ring slots that the real first step still reads
+            self.parents.fill_(-2)
             self._body()
             for t, v in zip(kept, saved):
                 t.copy_(v)
