@@ -51,3 +51,21 @@ def test_capturing_a_step_leaves_the_state_as_it_is(name):
         assert run.drawn.tolist() == [6] * 3 and torch.equal(run.st.pos, pos + 6)
     _close(graph.logits, eager.logits)
     m.engine.check_status()
+
+
+def test_a_row_that_has_stopped_keeps_its_cache():
+    """Row 0 stops in the first step, row 1 goes on: nothing of row 0 moves any more, whatever its ring has room for."""
+    m = _model("tiny")
+    V, n, eos = m.cfg.vocab_size, m.cfg.window + 9, 9
+    r = np.random.default_rng(3)
+    words = torch.zeros(2, (V + 31) // 32, dtype=torch.int32, device=DEV)
+    words[0, 0], words[1, 0] = 1 << eos, 1 << 7
+    run = _runner(m, [r.integers(20, V, n - 4).tolist() + [t] * 4 for t in (eos, 7)], 30, branches=1, depth=5, seed=1, eos_id=eos, allowed=words)
+    run.step()
+    assert run.done.tolist() == [True, False]
+    before, pos = _caches(run.st, slice(0, 1)), run.st.pos.clone()
+    for _ in range(3):
+        run.step()
+    assert _same(_caches(run.st, slice(0, 1)), before) and int(run.st.pos[0]) == int(pos[0]) and int(run.st.pos[1]) > int(pos[1])
+    run.run()
+    assert run.completions() == [[eos], [7] * 30]

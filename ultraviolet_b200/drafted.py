@@ -62,7 +62,7 @@ class TreeRunner:
             raise ValueError("a tree has at most 64 nodes: the last token and branches * depth drafted ones")
         if text.shape[0] != B or prompt_lengths.shape != (B,):
             raise ValueError(f"one text and one prompt length for each of {B} rows")
-        # (a row that has stopped, up to T tokens behind the last one wanted, still tries its last tree until all have)
+        # (a row's last tree may end T tokens behind the last one wanted; the other T are room for one more tree behind it)
         if st.max_len < text.size(1) + int(max_new) + 2 * self.T:
             raise ValueError(f"the state has {st.max_len} slots a row; {text.size(1)} + {max_new} tokens in trees of {self.T} need "
                              f"{text.size(1) + int(max_new) + 2 * self.T}")
@@ -77,7 +77,6 @@ class TreeRunner:
         self.length = self.prompt - 1                      # tokens in front of the root
         self.drawn = torch.zeros(B, dtype=torch.int64, device=dev)
         self.done = torch.zeros(B, dtype=torch.bool, device=dev)
-        self.pos_out = torch.empty_like(st.pos)
         self.tok, self.parents = self._drafts()
         M, V = B * self.T, eng.cfg.vocab_size
         row = lambda v: None if v is None else v if isinstance(v, Tensor) else torch.full((B,), float(v), dtype=torch.float32, device=dev)
@@ -92,9 +91,12 @@ class TreeRunner:
 
     def _drafts(self):
         if self.branches == 0:
-            root = self.text.gather(1, self.length[:, None]).long()
-            return root, torch.full((root.size(0), 1), -1, dtype=torch.int32, device=root.device)
-        return lookup_drafts(self.text[:, :self.cap], self.length, self.branches, self.depth)
+            tok = self.text.gather(1, self.length[:, None]).long()
+            parents = torch.full((tok.size(0), 1), -1, dtype=torch.int32, device=tok.device)
+        else:
+            tok, parents = lookup_drafts(self.text[:, :self.cap], self.length, self.branches, self.depth)
+        # a row that has stopped gets a tree without nodes: it draws nothing, and nothing of it moves
+        return tok, torch.where(self.done[:, None], -2, parents)
 
     def _body(self) -> None:
         st, eng, T = self.st, self.eng, self.T
@@ -106,11 +108,8 @@ class TreeRunner:
         steps = tree_positions(self.parents, self.drawn).view(-1)
         eng.sample(self.logits.view(B * T, -1), self.temperature, self.top_p, seed=self.seed, row_keys=self.row_keys, steps=steps,
                    tok_out=self.target, logp_out=self.logp, precapped=True, top_k=self.top_k)
-        _, count, new = eng.tree_advance(self.tok, self.target.view(B, T), self.parents, st, pos_out=self.pos_out)
-        # rows that had stopped before stay where they are
+        _, count, new = eng.tree_advance(self.tok, self.target.view(B, T), self.parents, st)
         j = torch.arange(T, device=new.device)
-        count = torch.where(self.done, 0, count.long())
-        st.pos.copy_(torch.where(self.done, st.pos, self.pos_out))
         live = j < count[:, None]
         self.text.scatter_(1, torch.where(live, self.length[:, None] + 1 + j, self.cap), new.to(torch.int32))
         self.length += count
