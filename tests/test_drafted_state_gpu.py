@@ -69,3 +69,15 @@ def test_a_row_that_has_stopped_keeps_its_cache():
     assert _same(_caches(run.st, slice(0, 1)), before) and int(run.st.pos[0]) == int(pos[0]) and int(run.st.pos[1]) > int(pos[1])
     run.run()
     assert run.completions() == [[eos], [7] * 30]
+
+
+@pytest.mark.parametrize("branches,depth", [(0, 1), (1, 4), (2, 3)])
+@pytest.mark.parametrize("kind", ["frequency", "presence"])
+def test_the_prompts_last_token_is_not_a_drawn_one(kind, branches, depth):
+    """Penalties for drawn tokens leave the first draw free to repeat the prompt's last token, and no later one."""
+    m = _model("tiny")
+    prompts = [[3, 4, 5, 3, 4, 5, 3, 4], [7], [2, 9, 2, 9, 2]]
+    for p in prompts:
+        a = p[-1]
+        out = generate_drafted(m, [p], 6, group=2, branches=branches, depth=depth, temperature=0.0, logit_bias={a: 500.0}, **{kind: 1000.0})
+        assert all(r[0] == a and a not in r[1:] for r in out[0]), out

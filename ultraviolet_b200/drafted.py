@@ -103,8 +103,11 @@ class TreeRunner:
         B = st.B
         h = eng.tree_trunk(self.tok, self.parents, st)
         torch.mm(h, eng.w["embed"].t(), out=self.head)
-        adjust_logits(self.head.view(B, T, -1), softcap=eng.cfg.softcap, history=self.text, lengths=self.length,
-                      prompt_lengths=self.prompt, parents=self.parents, tokens=self.tok, out=self.logits, **self.adjust)
+        # the root stands in the text, where it counts as what it is: in the first step as the prompt's last token, then as a drawn one
+        drafted = self.tok.clone()
+        drafted[:, 0] = -1
+        adjust_logits(self.head.view(B, T, -1), softcap=eng.cfg.softcap, history=self.text, lengths=self.length + 1,
+                      prompt_lengths=self.prompt, parents=self.parents, tokens=drafted, out=self.logits, **self.adjust)
         steps = tree_positions(self.parents, self.drawn).view(-1)
         eng.sample(self.logits.view(B * T, -1), self.temperature, self.top_p, seed=self.seed, row_keys=self.row_keys, steps=steps,
                    tok_out=self.target, logp_out=self.logp, precapped=True, top_k=self.top_k)
