@@ -81,3 +81,32 @@ def test_the_prompts_last_token_is_not_a_drawn_one(kind, branches, depth):
         a = p[-1]
         out = generate_drafted(m, [p], 6, group=2, branches=branches, depth=depth, temperature=0.0, logit_bias={a: 500.0}, **{kind: 1000.0})
         assert all(r[0] == a and a not in r[1:] for r in out[0]), out
+
+
+def test_steps_of_two_states_do_not_meet():
+    """tree_step on one state, tree_step on another, then both accepts: each state takes its own nodes."""
+    m = _model("tiny")
+    V, T = m.cfg.vocab_size, 5
+    g = torch.Generator(device=DEV).manual_seed(5)
+    parents = torch.arange(-1, T - 1, device=DEV, dtype=torch.int32)
+    idx = [np.random.default_rng(i).integers(1, V, (3, 6)) for i in range(2)]
+    tok = [torch.randint(0, V, (3, T), generator=g, device=DEV) for _ in range(2)]
+    target = [torch.cat([t[:, 1:], t[:, :1]], 1) for t in tok]                    # all of it is accepted
+    new = lambda: [_prefilled(m, i, np.zeros(3, np.int64), 40) for i in idx]
+    apart, mixed = new(), new()
+    for st, t, y in zip(apart, tok, target):
+        m.tree_step(t, parents, st)
+        m.tree_accept(t, y, parents, st)
+    for st, t in zip(mixed, tok):
+        m.tree_step(t, parents, st)
+    for st, t, y in zip(mixed, tok, target):
+        m.tree_accept(t, y, parents, st)
+    for a, b in zip(apart, mixed):
+        assert torch.equal(a.pos, b.pos) and int(a.pos.min()) == 6 + T and _same(_caches(a), _caches(b))
+    # an accept without its step, or of a step of another shape
+    st = new()[0]
+    with pytest.raises(RuntimeError):
+        m.tree_accept(tok[0], target[0], parents, st)
+    m.tree_step(tok[0], parents, st)
+    with pytest.raises(RuntimeError):
+        m.tree_accept(tok[0][:, :3], target[0][:, :3], parents[:3], st)

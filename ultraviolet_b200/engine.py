@@ -82,7 +82,6 @@ class DecodeEngine:
         if cfg.rope_pairs:
             self.inv_freq.copy_((1.0 / cfg.rope_base) ** torch.linspace(0, 1, cfg.rope_pairs, dtype=torch.float32))
         self._scratch: dict[int, dict] = {}
-        self._tree_qkv: dict[int, Tensor] = {}
         self._prefill_trunk = self._prefill_flags = self._prefill_oob = None
         self._fuse_plan = None      # load_from's launch arguments for the parameter tensors it saw last
         self._fuse_status = torch.zeros(1, dtype=torch.int32, device=self.device)
@@ -658,15 +657,6 @@ class DecodeEngine:
         _lib.check(lib.uv_prefill_attn(C.byref(pa), sp), "uv_prefill_attn")
 
     # ------------------------------------------------------------------------------------------------ drafted tokens
-    def tree_qkv(self, M: int) -> Tensor:
-        """(n_layers, M, (H + 2K) * hd): the projections of the nodes of a tree step, until tree_advance has taken the accepted ones."""
-        t = self._tree_qkv.get(M)
-        if t is None:
-            cfg = self.cfg
-            t = self._tree_qkv[M] = torch.empty(cfg.n_layers, M, (cfg.n_heads + 2 * cfg.n_kv_heads) * cfg.head_dim, dtype=self.dtype,
-                                                device=self.device)
-        return t
-
     def tree_trunk(self, tok: Tensor, parents: Tensor, st) -> Tensor:
         """One step of trees of drafted tokens: tok (B, T), parents (B, T) or (T,) (kernels.tree_attention's), row b of the state
         at st.pos[b].  Returns the final normed hidden (B * T, d), a view of engine scratch; the state stays as it is."""
@@ -677,14 +667,15 @@ class DecodeEngine:
         pos = st.pos[:B]
         nodes = tree_positions(parents, pos).view(-1)
         return self.trunk(tok.reshape(-1), st, nodes, nodes,
-                          tree=dict(parents=parents, pos=pos, starts=st.starts[:B], qkv=self.tree_qkv(B * T)))
+                          tree=dict(parents=parents, pos=pos, starts=st.starts[:B], qkv=st.tree_nodes(B, T, self.dtype)))
 
     def tree_advance(self, tok: Tensor, target: Tensor, parents: Tensor, st, pos_out: Tensor | None = None):
-        """kernels.tree_advance behind tree_trunk: the accepted path of every tree, with its keys and values in the state's caches."""
+        """kernels.tree_advance behind tree_trunk on the same state: the accepted path of every tree, with its keys and values in the
+        state's caches."""
         from .kernels.tree import tree_advance
         cfg, (B, T) = self.cfg, tok.shape
         H, K = cfg.n_heads, cfg.n_kv_heads
-        qkv = self.tree_qkv(B * T).view(cfg.n_layers, B, T, H + 2 * K, cfg.head_dim)
+        qkv = st.tree_nodes(B, T).view(cfg.n_layers, B, T, H + 2 * K, cfg.head_dim)
         return tree_advance(qkv[:, :, :, H:H + K].unbind(0), qkv[:, :, :, H + K:].unbind(0), st.k, st.v, st.k_scale, st.v_scale, st.rings,
                             parents, tok, target, st.pos[:B], pos_out=pos_out, oob=self.scratch(B * T)["oob"])
 

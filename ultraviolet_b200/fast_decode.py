@@ -54,6 +54,8 @@ class KernelDecodeState:
         self.starts = torch.zeros(B, dtype=torch.long, device=device)
         self.host_pos = np.zeros(B, dtype=np.int64)
         self.prev = None
+        self._tree_nodes: dict[tuple[int, int], Tensor] = {}
+        self._tree_shape = None
 
     def set_pos(self, p: int):
         self.pos.fill_(p)
@@ -73,6 +75,22 @@ class KernelDecodeState:
         pairs = torch.from_numpy(np.stack([src, dst])).to(self.pos.device)
         kv_fork(self.k, self.v, self.k_scale, self.v_scale, self.rings, pairs[0], pairs[1], self.pos, self.starts)
         self.host_pos[dst] = self.host_pos[src]
+
+    def tree_nodes(self, B: int, T: int, dtype=None) -> Tensor:
+        """(n_layers, B * T, (H + 2K) * hd): the projections of the nodes of a step of B trees of T nodes, which stay here until the
+        accepted ones are taken into the caches.  With a dtype: for a step to fill; without: what the last step left."""
+        if dtype is None:
+            if self._tree_shape != (B, T):
+                raise RuntimeError(f"{B} trees of {T} nodes are accepted on a state whose last step was " +
+                                   ("none" if self._tree_shape is None else "of {} trees of {} nodes".format(*self._tree_shape)))
+            return self._tree_nodes[B, T]
+        self._tree_shape = B, T
+        t = self._tree_nodes.get((B, T))
+        if t is None or t.dtype != dtype:
+            cfg = self.cfg
+            t = self._tree_nodes[B, T] = torch.empty(cfg.n_layers, B * T, (cfg.n_heads + 2 * cfg.n_kv_heads) * cfg.head_dim, dtype=dtype,
+                                                     device=self.pos.device)
+        return t
 
     def nbytes(self) -> int:
         ts = self.k + self.v + self.k_scale + self.v_scale
@@ -115,7 +133,7 @@ def tree_step_fast(self, tok: Tensor, parents: Tensor, st: KernelDecodeState, re
 
 @torch.no_grad()
 def tree_accept_fast(self, tok: Tensor, target: Tensor, parents: Tensor, st: KernelDecodeState):
-    """The end of the step that ``tree_step_fast`` began with the same tok and parents: target (B, T) holds the token drawn
+    """The end of the step that ``tree_step_fast`` began with the same tok, parents and st: target (B, T) holds the token drawn
     behind every node, the caches take the accepted path, st.pos advances by its length.  Returns kernels.tree_advance's
     (path, count, drawn).  (st.host_pos, which the host alone advances, is left behind.)"""
     return _engine(self).tree_advance(tok, target, parents, st)
