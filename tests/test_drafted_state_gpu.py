@@ -110,3 +110,31 @@ def test_steps_of_two_states_do_not_meet():
     m.tree_step(tok[0], parents, st)
     with pytest.raises(RuntimeError):
         m.tree_accept(tok[0][:, :3], target[0][:, :3], parents[:3], st)
+
+
+def test_tokens_of_any_layout():
+    m = _model("tiny")
+    V = m.cfg.vocab_size
+    idx = np.random.default_rng(1).integers(1, V, (4, 6))
+    st = _prefilled(m, idx, np.zeros(4, np.int64), 40)
+    text = torch.randint(0, V, (4, 9), generator=torch.Generator(device=DEV).manual_seed(2), device=DEV)
+    one, two = torch.tensor([-1], device=DEV), torch.tensor([-1, 0], device=DEV)
+    for tok, parents in ((text[:, -1:], one), (text[:, 2:7:4], two), (text.t()[:2].t(), two)):
+        assert torch.equal(m.tree_step(tok, parents, st), m.tree_step(tok.contiguous(), parents, st))
+
+
+def test_tokens_of_any_integer_type_and_no_others():
+    m = _model("tiny")
+    idx = np.random.default_rng(1).integers(1, m.cfg.vocab_size, (4, 6))
+    st = _prefilled(m, idx, np.zeros(4, np.int64), 40)
+    tok = torch.randint(0, 100, (4, 2), generator=torch.Generator(device=DEV).manual_seed(2), device=DEV)
+    parents = torch.tensor([-1, 0], device=DEV)
+    want = m.tree_step(tok, parents, st)
+    for dtype in (torch.int32, torch.int16, torch.uint8):
+        assert torch.equal(m.tree_step(tok.to(dtype), parents, st), want)
+    with pytest.raises(ValueError):
+        m.tree_step(tok.float(), parents, st)
+    with pytest.raises(ValueError):
+        m.tree_step(tok.flatten(), parents, st)
+    with pytest.raises(RuntimeError):
+        m.tree_step(tok.cpu(), parents, st)

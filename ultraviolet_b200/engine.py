@@ -660,13 +660,18 @@ class DecodeEngine:
     def tree_trunk(self, tok: Tensor, parents: Tensor, st) -> Tensor:
         """One step of trees of drafted tokens: tok (B, T), parents (B, T) or (T,) (kernels.tree_attention's), row b of the state
         at st.pos[b].  Returns the final normed hidden (B * T, d), a view of engine scratch; the state stays as it is."""
+        from .kernels._util import need_cuda
         from .kernels.tree import tree_positions
+        need_cuda(tok, st.pos)
+        if tok.dim() != 2 or tok.is_floating_point() or tok.is_complex() or tok.dtype == torch.bool:
+            raise ValueError(f"tok has to hold integers (B, T); got {tuple(tok.shape)} {tok.dtype}")
         B, T = tok.shape
         if B > st.B:
             raise ValueError(f"{B} trees for a state of {st.B} rows")
+        tok = tok.to(torch.int64).contiguous().view(-1)         # as the kernels read it
         pos = st.pos[:B]
         nodes = tree_positions(parents, pos).view(-1)
-        return self.trunk(tok.reshape(-1), st, nodes, nodes,
+        return self.trunk(tok, st, nodes, nodes,
                           tree=dict(parents=parents, pos=pos, starts=st.starts[:B], qkv=st.tree_nodes(B, T, self.dtype)))
 
     def tree_advance(self, tok: Tensor, target: Tensor, parents: Tensor, st, pos_out: Tensor | None = None):
