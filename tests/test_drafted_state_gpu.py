@@ -138,3 +138,14 @@ def test_tokens_of_any_integer_type_and_no_others():
         m.tree_step(tok.flatten(), parents, st)
     with pytest.raises(RuntimeError):
         m.tree_step(tok.cpu(), parents, st)
+
+
+def test_a_tree_of_another_width_is_refused():
+    """Before anything is launched: the step would read positions that the tree does not have."""
+    m = _model("tiny")
+    idx = np.random.default_rng(1).integers(1, m.cfg.vocab_size, (2, 6))
+    st = _prefilled(m, idx, np.zeros(2, np.int64), 40)
+    tok = torch.zeros((2, 4), dtype=torch.int64, device=DEV)
+    for parents in ([-1], [-1, 0, 0], [-1, 0, 0, 0, 0], [[-1, 0, 0, 0]], [[-1, 0, 0]] * 2, [[-1, 0, 0, 0]] * 3):
+        with pytest.raises(ValueError):
+            m.tree_step(tok, torch.tensor(parents, device=DEV), st)

@@ -668,6 +668,8 @@ class DecodeEngine:
         B, T = tok.shape
         if B > st.B:
             raise ValueError(f"{B} trees for a state of {st.B} rows")
+        if tuple(parents.shape) not in ((B, T), (T,)):          # (the nodes' positions are made from it, one for each token)
+            raise ValueError(f"parents have to be ({B}, {T}) or ({T},); got {tuple(parents.shape)}")
         tok = tok.to(torch.int64).contiguous().view(-1)         # as the kernels read it
         pos = st.pos[:B]
         nodes = tree_positions(parents, pos).view(-1)
