@@ -149,3 +149,12 @@ def test_a_tree_of_another_width_is_refused():
     for parents in ([-1], [-1, 0, 0], [-1, 0, 0, 0, 0], [[-1, 0, 0, 0]], [[-1, 0, 0]] * 2, [[-1, 0, 0, 0]] * 3):
         with pytest.raises(ValueError):
             m.tree_step(tok, torch.tensor(parents, device=DEV), st)
+
+
+def test_prompt_lengths_that_the_text_does_not_have():
+    m = _model("tiny")
+    text = torch.ones(2, 4, dtype=torch.int32, device=DEV)
+    for lens in ([0, 4], [4, 5], [-1, 2]):
+        for where in ("cpu", DEV):
+            with pytest.raises(ValueError):
+                TreeRunner(m, m.new_state(2, 64), text, torch.tensor(lens, device=where), 8, 1, 3)

@@ -62,6 +62,8 @@ class TreeRunner:
             raise ValueError("a tree has at most 64 nodes: the last token and branches * depth drafted ones")
         if text.shape[0] != B or prompt_lengths.shape != (B,):
             raise ValueError(f"one text and one prompt length for each of {B} rows")
+        if B and not (1 <= int(prompt_lengths.min()) and int(prompt_lengths.max()) <= text.size(1)):   # (they index the text)
+            raise ValueError(f"prompts have 1 to {text.size(1)} tokens, as the text does")
         # (a row's last tree may end T tokens behind the last one wanted; the other T are room for one more tree behind it)
         if st.max_len < text.size(1) + int(max_new) + 2 * self.T:
             raise ValueError(f"the state has {st.max_len} slots a row; {text.size(1)} + {max_new} tokens in trees of {self.T} need "
