@@ -158,3 +158,11 @@ def test_prompt_lengths_that_the_text_does_not_have():
         for where in ("cpu", DEV):
             with pytest.raises(ValueError):
                 TreeRunner(m, m.new_state(2, 64), text, torch.tensor(lens, device=where), 8, 1, 3)
+
+
+def test_allowed_tokens_outside_the_vocabulary_allow_nothing():
+    m = _model("tiny")
+    V = m.cfg.vocab_size
+    out = generate_drafted(m, [[1, 2, 3]], 5, branches=1, depth=3, temperature=0.0, allowed_ids=[7, -1, V, V + 31, 2 ** 40],
+                           logit_bias={V - 1: 1e4})
+    assert out == [[[7] * 5]]

@@ -203,7 +203,8 @@ def generate_drafted(model, prompts, max_new: int, group: int = 1, branches: int
         bias = torch.tensor([float(v) for v in logit_bias.values()], dtype=torch.float32, device=dev)
     if allowed_ids is not None:
         bits = torch.zeros((V + 31) // 32 * 32, dtype=torch.int64)
-        bits[torch.as_tensor(list(allowed_ids), dtype=torch.int64)] = 1
+        ids = torch.as_tensor(list(allowed_ids), dtype=torch.int64)
+        bits[ids[(ids >= 0) & (ids < V)]] = 1                   # (others are no tokens: ignored, as adjust_logits does)
         words = (bits.view(-1, 32) << torch.arange(32)).sum(1)
         allowed = torch.where(words >= 2 ** 31, words - 2 ** 32, words).to(torch.int32).to(dev).expand(B, -1)
     runner = TreeRunner(model, st, text.repeat_interleave(group, 0).to(dev), lens.repeat_interleave(group), max_new, branches, depth,
