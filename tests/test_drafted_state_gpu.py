@@ -166,3 +166,10 @@ def test_allowed_tokens_outside_the_vocabulary_allow_nothing():
     out = generate_drafted(m, [[1, 2, 3]], 5, branches=1, depth=3, temperature=0.0, allowed_ids=[7, -1, V, V + 31, 2 ** 40],
                            logit_bias={V - 1: 1e4})
     assert out == [[[7] * 5]]
+
+
+def test_the_hosts_positions_follow_a_run():
+    m = _model("tiny")
+    run = _runner(m, [[1, 2, 3, 4], [4, 3, 2, 1]], 12, branches=1, depth=3, temperature=0.0)
+    run.run()
+    assert run.st.host_pos.tolist() == run.st.pos.tolist() and int(run.st.pos.min()) >= 3 + 12

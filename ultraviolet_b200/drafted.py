@@ -159,6 +159,7 @@ class TreeRunner:
         while not bool(self.done.all()):
             for _ in range(check_every):
                 self.step()
+        self.st.host_pos[:] = self.st.pos.cpu().numpy()         # (what goes on with the state plans by it)
         self.eng.check_status(self.st.B * self.T)
 
     def completions(self) -> list[list[int]]:
