@@ -94,6 +94,7 @@ __global__ void __launch_bounds__(TR_THREADS) tree_rows_kernel(const __grid_cons
   const bool producer = warp == TR_WARPS;
   const int b = blockIdx.x / a.KH, kh = blockIdx.x % a.KH, sid = blockIdx.y, row0 = blockIdx.z * ROWS;
   const int rows = min(ROWS, P.M - row0);
+  pdl_wait();     // positions, queries, the nodes' keys and values and the caches come from the kernels before this one
 
   // ---- the part's tiles
   const RowRange rg = row_range(a, b);
