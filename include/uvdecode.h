@@ -546,8 +546,9 @@ int uv_tree_positions(const int32_t* parents, int64_t parents_stride, const int6
  * the ancestors j with depth_i - depth_j < window (window 0 = unlimited).  The nodes' keys and values go through the cache's
  * quantiser first, so they are the numbers that uv_tree_advance will append: a tree step reads what the same tokens
  * would read one at a time.  out[b, i, h] = softmax(scale * q . K) V with fp32 statistics, rounded once; then the optional
- * epilogue of uv_attn_args (XSA with the node's own unquantised v, head gates).  A node that is absent or sees nothing
- * gets zeros.  head_dim 16, 32, 64 or 128, at most 16 query heads per kv head.
+ * epilogue of uv_attn_args (XSA with the node's own unquantised v, head gates).  An absent node gets zeros; a present one
+ * sees itself at least, and gets NaN where its query is not finite or a scale that it sees is no number.  head_dim 16, 32, 64
+ * or 128, at most 16 query heads per kv head.
  *
  * num_splits: 0 lets the library choose; n >= 1 cuts each row's keys into n parts (few query rows only).  Partials go through
  * workspace: uv_tree_attn_workspace_bytes(args) bytes, 16-byte aligned (0: none needed).  status as in uv_attn_args. */

@@ -1,0 +1,70 @@
+"""Values and layouts at which the tree kernels have to agree with their formulas and with each other."""
+import pytest
+import torch
+
+from oracle import tree as ot
+from tests.test_tree_gpu import UNIT, _gen, _np, _state, _tree
+
+pytestmark = pytest.mark.gpu
+
+# one call for each way through the kernels: B, T, H, K, hd, S, num_splits
+ROUTES = {
+    "rows, whole": (3, 3, 8, 1, 64, 90, 1),
+    "rows, parts in a cluster": (3, 6, 8, 1, 64, 700, 4),
+    "rows, parts in the workspace": (3, 5, 8, 2, 128, 2000, 12),
+    "rows, plain copies": (3, 4, 4, 2, 32, 91, 1),
+    "128 rows a unit, whole": (90, 16, 8, 1, 64, 130, None),
+    "128 rows a unit, cut": (3, 40, 8, 1, 64, 60000, None),
+    "two tiles at a time, whole": (256, 8, 8, 1, 64, 500, None),
+    "two tiles at a time, cut": (16, 5, 8, 1, 64, 70000, None),
+    "head_dim 128, cut": (4, 40, 8, 2, 128, 30000, None),
+}
+
+
+def _call(route, dtype=torch.bfloat16, kind="random"):
+    from ultraviolet_b200.kernels import tree_attention
+    B, T, H, K, hd, S, splits = ROUTES[route]
+    kc, vc, ks, vs = _state(B, K, S, hd, dtype, T)
+    x = torch.randn((B, T, H + 2 * K, hd), generator=_gen(T), device="cuda").to(dtype)
+    pos = torch.arange(B, device="cuda") * 7 % 30 + (S - 30)
+    par = torch.tensor(_tree(kind, B, T, T), device="cuda")
+
+    def run(x, ks=ks, vs=vs, **kw):
+        return tree_attention(x[:, :, :H], x[:, :, H:H + K], x[:, :, H + K:], kc, vc, pos, pos * 0, par, 0.14, k_scale=ks, v_scale=vs,
+                              num_splits=splits, **kw)
+    return run, x, ks, vs, pos, par
+
+
+@pytest.mark.parametrize("route", sorted(ROUTES))
+def test_what_is_not_finite_shows(route):
+    """A present node whose query, or a visible key's scale, is no number has no softmax: NaN on every route, and nothing else changes."""
+    B, T, H, K, hd, S, splits = ROUTES[route]
+    run, x, ks, vs, pos, par = _call(route)
+    want = run(x)
+    y = x.clone()
+    hit = [(0, T - 1, 1, float("nan")), (1, 0, 0, float("inf")), (2, 1, H - 1, float("-inf"))]
+    for b, t, h, v in hit:
+        y[b, t, h, 3] = v
+    y[0, 1, 2] = float("nan")
+    hit.append((0, 1, 2, None))
+    got, keep = run(y), torch.ones_like(want[..., 0], dtype=torch.bool)
+    for b, t, h, _ in hit:
+        assert got[b, t, h].isnan().all(), (b, t, h)
+        keep[b, t, h] = False
+    assert torch.equal(got[keep], want[keep])
+    # a visible key's scale: all nodes of that row, and of the kv head's query heads
+    bad = ks.clone()
+    bad[1, K - 1, S // 2] = float("nan")
+    got, keep = run(x, ks=bad), torch.ones_like(want[..., 0], dtype=torch.bool)
+    keep[1, :, H - H // K:] = False
+    assert got[~keep].isnan().all() and torch.equal(got[keep], want[keep])
+
+
+@pytest.mark.parametrize("route", sorted(ROUTES))
+def test_absent_nodes_get_zeros_whatever_they_hold(route):
+    run, x, ks, vs, pos, par = _call(route, kind="padded")
+    par[:, 1] = -2
+    y = x.clone()
+    y[:, 1] = float("nan")
+    want, got = run(x), run(y)
+    assert (got[:, 1] == 0).all() and torch.equal(got, want)

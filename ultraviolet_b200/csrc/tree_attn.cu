@@ -485,14 +485,14 @@ __global__ void __launch_bounds__(TR_THREADS) tree_rows_kernel(const __grid_cons
 #pragma unroll
       for (int w = 0; w < TR_WARPS; ++w) {
         const float wt = mw[w] == -INFINITY ? 0.f : ex2(mw[w] - mx);          // (what a warp without keys holds is zeros)
-        lsum += wt * mg_l[w * ROWS + row];
+        lsum += part_sum(mw[w], wt, mg_l[w * ROWS + row]);
 #pragma unroll
         for (int i = 0; i < EPL; ++i)
           if (HD >= 32 || lane < HD) z[i] += wt * mg_o[(w * ROWS + row) * HD + lane + 32 * i];
       }
     }
     if (P.splits == 1) {
-      const float inv = lsum > 0.f ? 1.0f / lsum : 0.f;
+      const float inv = inverse_sum(lsum);
 #pragma unroll
       for (int i = 0; i < EPL; ++i) z[i] *= inv;
       store_row<QT, HD>(P, z, b, kh, row0 + row, sets.mask[node_of(P, row0 + row)] != 0, lane);
@@ -515,7 +515,7 @@ __global__ void __launch_bounds__(TR_THREADS) tree_rows_kernel(const __grid_cons
   for (int row = sid + warp * P.splits; row < rows; row += (TR_WARPS + 1) * P.splits) {
     float m_s = -INFINITY, l_s = 0.f, z[EPL];
     if (lane < P.splits) m_s = peer_f32(pm + row * 4u, lane), l_s = peer_f32(pl + row * 4u, lane);
-    const float mx = warp_max(m_s), wt_s = m_s == -INFINITY ? 0.f : ex2(m_s - mx), lsum = warp_sum(wt_s * l_s);
+    const float mx = warp_max(m_s), wt_s = m_s == -INFINITY ? 0.f : ex2(m_s - mx), lsum = warp_sum(part_sum(m_s, wt_s, l_s));
 #pragma unroll
     for (int i = 0; i < EPL; ++i) z[i] = 0.f;
 #pragma unroll 4
@@ -525,7 +525,7 @@ __global__ void __launch_bounds__(TR_THREADS) tree_rows_kernel(const __grid_cons
       for (int i = 0; i < EPL; ++i)
         if (HD >= 32 || lane < HD) z[i] += wt * peer_f32(po + (uint32_t)(row * HD + lane + 32 * i) * 4u, s);
     }
-    const float inv = lsum > 0.f ? 1.0f / lsum : 0.f;
+    const float inv = inverse_sum(lsum);
 #pragma unroll
     for (int i = 0; i < EPL; ++i) z[i] *= inv;
     store_row<QT, HD>(P, z, b, kh, row0 + row, sets.mask[node_of(P, row0 + row)] != 0, lane);
@@ -552,18 +552,16 @@ __global__ void __launch_bounds__(128) tree_combine_kernel(const __grid_constant
   mx = warp_max(mx);
 #pragma unroll
   for (int i = 0; i < EPL; ++i) z[i] = 0.f;
-  if (mx != -INFINITY)
-    for (int s = 0; s < P.splits; ++s) {
-      const int64_t w = w0 + (int64_t)s * P.M;
-      const float m = P.ws_m[w];
-      if (m == -INFINITY) continue;
-      const float wt = ex2(m - mx);
-      lsum += wt * P.ws_l[w];
+  for (int s = 0; s < P.splits; ++s) {
+    const int64_t w = w0 + (int64_t)s * P.M;
+    const float m = P.ws_m[w], wt = m == -INFINITY ? 0.f : ex2(m - mx);
+    lsum += part_sum(m, wt, P.ws_l[w]);
+    if (m == -INFINITY) continue;
 #pragma unroll
-      for (int i = 0; i < EPL; ++i)
-        if (HD >= 32 || lane < HD) z[i] += wt * P.ws_o[w * HD + lane + 32 * i];
-    }
-  const float inv = lsum > 0.f ? 1.0f / lsum : 0.f;
+    for (int i = 0; i < EPL; ++i)
+      if (HD >= 32 || lane < HD) z[i] += wt * P.ws_o[w * HD + lane + 32 * i];
+  }
+  const float inv = inverse_sum(lsum);
 #pragma unroll
   for (int i = 0; i < EPL; ++i) z[i] *= inv;
   store_row<QT, HD>(P, z, b, kh, row, par[up] == -1, lane);

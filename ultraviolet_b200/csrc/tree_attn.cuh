@@ -55,6 +55,12 @@ __device__ __forceinline__ RowRange row_range(const uv_tree_attn_args& a, int b)
   return r;
 }
 
+// ---- 1 / sum of a row's weights.  A present node sees itself at least, so its sum is positive unless its query is not finite or a
+//      scale that it sees is no number: then there is no softmax, and NaN says so.
+__device__ __forceinline__ float inverse_sum(float sum) { return sum > 0.f ? 1.0f / sum : __int_as_float(0x7fffffff); }
+// a part's sum in a merge, weighted: one without a reference has seen no score that is a number, and its sum is 0 or NaN
+__device__ __forceinline__ float part_sum(float m, float weight, float sum) { return m == -INFINITY ? sum : weight * sum; }
+
 // ---- epilogue of one query row held by a warp (lane owns dims lane + 32 i), and its store
 template <typename QT, int HD>
 __device__ __forceinline__ void store_row(const TreeParams& P, float (&z)[(HD + 31) / 32], int b, int kh, int row, bool present,

@@ -789,11 +789,11 @@ __global__ void __launch_bounds__(TT_THREADS, TcSmem<HD>::CTAS) tree_tc_kernel(c
       }
       soft_bar();
       const bool dead = sh.dead != 0, whole_unit = n == pc.n;
-      float row_m = sh.m[trow], row_l = dead ? 0.f : sh.l[trow], share = 1.0f;         // (dead: zeros, and the status word)
+      float row_m = sh.m[trow], row_l = dead ? 0.f : sh.l[trow], share = 1.0f;         // (dead: NaN, and the status word)
       if (DUAL) {                                                 // both lanes of a row get what the two have seen
         const float both = fmaxf(row_m, __shfl_xor_sync(0xffffffffu, row_m, 16));
         share = row_m == -INFINITY ? 0.f : ex2(row_m - both);
-        row_l *= share;
+        row_l = part_sum(row_m, share, row_l);
         row_l += __shfl_xor_sync(0xffffffffu, row_l, 16);
         row_m = both;
       }
@@ -818,7 +818,7 @@ __global__ void __launch_bounds__(TT_THREADS, TcSmem<HD>::CTAS) tree_tc_kernel(c
       const int64_t to = ((int64_t)2 * cta + (t0 == 0 ? 1 : 0)) * TT_ROWS + row_at(trow);
       if (!whole_unit && slab == 0 && writes) ws_ml[2 * to] = dead ? -INFINITY : row_m, ws_ml[2 * to + 1] = row_l;
       if (row0 + row_of_lane(32 * quad) < P.M) {
-        const float inv = whole_unit ? (row_l > 0.f ? 1.0f / row_l : 0.f) : 1.0f;
+        const float inv = whole_unit ? inverse_sum(row_l) : 1.0f;
         const uint4* v = reinterpret_cast<const uint4*>(static_cast<const QT*>(a.v) + (int64_t)b * a.snvb + (int64_t)t * a.snvt + (int64_t)kh * a.snvh);
         float xs = 0.f;                            // XSA: z - xs * v
         const bool xsa = whole_unit && a.xsa_alpha != nullptr;
@@ -898,19 +898,17 @@ __global__ void __launch_bounds__(256) tree_tc_merge_kernel(const __grid_constan
   float lsum = 0.f, z[EPL];
 #pragma unroll
   for (int i = 0; i < EPL; ++i) z[i] = 0.f;
-  if (mx != -INFINITY)
 #pragma unroll 2
-    for (int k = c.x; k <= c.y; ++k) {
-      const int64_t w = at(k);
-      const float m = ws_ml[2 * w];
-      if (m == -INFINITY) continue;
-      const float wt = ex2(m - mx);
-      lsum += wt * ws_ml[2 * w + 1];
+  for (int k = c.x; k <= c.y; ++k) {
+    const int64_t w = at(k);
+    const float m = ws_ml[2 * w], wt = m == -INFINITY ? 0.f : ex2(m - mx);
+    lsum += part_sum(m, wt, ws_ml[2 * w + 1]);
+    if (m == -INFINITY) continue;
 #pragma unroll
-      for (int i = 0; i < EPL; ++i)
-        if (HD >= 32 || lane < HD) z[i] += wt * ws_o[w * HD + lane + 32 * i];
-    }
-  const float inv = lsum > 0.f ? 1.0f / lsum : 0.f;
+    for (int i = 0; i < EPL; ++i)
+      if (HD >= 32 || lane < HD) z[i] += wt * ws_o[w * HD + lane + 32 * i];
+  }
+  const float inv = inverse_sum(lsum);
 #pragma unroll
   for (int i = 0; i < EPL; ++i) z[i] *= inv;
   store_row<QT, HD>(P, z, b, kh, row, par[up] == -1, lane);

@@ -59,8 +59,9 @@ def tree_attention(q: Tensor, k: Tensor, v: Tensor, k_cache: Tensor, v_cache: Te
     starts (B,) the first valid one.  A node at position p sees the cached positions max(starts, p - window + 1, 0) .. pos - 1
     (window 0: no limit; ring, default window > 0: the newest S of them, position t in slot t % S) and its ancestors within the
     window, itself included.  The nodes' keys and values pass through the cache's quantiser first: a step of a tree reads what
-    the same tokens would read one at a time.  row_map (B,): cache row of batch row b.  An absent node, or one that sees nothing, gets
-    zeros.  num_splits: parts into which a row's keys are cut (None: chosen by the library)."""
+    the same tokens would read one at a time.  row_map (B,): cache row of batch row b.  An absent node gets zeros; a present one sees
+    itself at least, and gets NaN where its query is not finite or a scale that it sees is no number.  num_splits: parts into which a row's
+    keys are cut (None: chosen by the library)."""
     scale, window, splits = float(scale), int(window), int(num_splits or 0)
     if not torch.compiler.is_compiling():
         out = _lib.host().tree_attention(q, k, v, k_cache, v_cache, pos, starts, parents, scale, k_scale, v_scale, window,
