@@ -68,3 +68,37 @@ def test_absent_nodes_get_zeros_whatever_they_hold(route):
     y[:, 1] = float("nan")
     want, got = run(x), run(y)
     assert (got[:, 1] == 0).all() and torch.equal(got, want)
+
+
+def test_watched_calls_count_what_they_skip():
+    from torch.utils._python_dispatch import TorchDispatchMode
+    from ultraviolet_b200.kernels import kv_fork, tree_advance
+
+    class Watch(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+
+    B, T, S = 3, 4, 20
+    kc, vc, ks, vs = _state(B, 1, S, 64, torch.bfloat16, 1)
+    x = torch.randn((B, T, 2, 64), generator=_gen(1), device="cuda").to(torch.bfloat16)
+    par, tok = torch.arange(-1, T - 1, device="cuda"), torch.zeros((B, T), dtype=torch.long, device="cuda")
+    new = lambda: torch.zeros(1, dtype=torch.int32, device="cuda")
+    dev = lambda *a: torch.tensor(a, device="cuda")
+
+    def advance(oob):
+        pos = dev(2, S - 1, 5)                       # row 1: three nodes behind the end of its cache; row 2: no cache row
+        tree_advance([x[:, :, :1]], [x[:, :, 1:]], [kc], [vc], [ks], [vs], [False], par, tok, tok, pos, row_map=dev(0, 1, B), oob=oob)
+        return pos
+
+    def fork(oob):
+        pos, starts = dev(4, 5, 6), dev(0, 0, 0)
+        kv_fork([kc], [vc], [ks], [vs], [False], dev(0, 0, -1), dev(1, B, 2), pos, starts, oob=oob)
+        return pos
+
+    for call, skipped in ((advance, 2 * 3 + 2 * T), (fork, 2)):
+        plain, watched = new(), new()
+        want = call(plain)
+        with Watch():
+            got = call(watched)
+            call(None)
+        assert torch.equal(got, want) and int(plain) == int(watched) == skipped

@@ -73,16 +73,17 @@ def tree_attention(q: Tensor, k: Tensor, v: Tensor, k_cache: Tensor, v_cache: Te
                          window > 0 if ring is None else bool(ring), row_map, splits)
 
 
-@torch.library.custom_op("uvb200::tree_advance", mutates_args=("k_caches", "v_caches", "k_scales", "v_scales", "pos_out"))
+@torch.library.custom_op("uvb200::tree_advance", mutates_args=("k_caches", "v_caches", "k_scales", "v_scales", "pos_out", "oob"))
 def _advance_op(k: Sequence[Tensor], v: Sequence[Tensor], k_caches: Sequence[Tensor], v_caches: Sequence[Tensor],
                 k_scales: Sequence[Tensor], v_scales: Sequence[Tensor], rings: Sequence[bool], parents: Tensor, tokens: Tensor,
-                target: Tensor, pos: Tensor, row_map: Optional[Tensor], pos_out: Tensor) -> tuple[Tensor, Tensor, Tensor]:
+                target: Tensor, pos: Tensor, row_map: Optional[Tensor], pos_out: Tensor,
+                oob: Optional[Tensor]) -> tuple[Tensor, Tensor, Tensor]:
     return _lib.host().tree_advance(k, v, k_caches, v_caches, k_scales, v_scales, list(rings), parents, tokens, target, pos, row_map,
-                                    pos_out, None, True)
+                                    pos_out, oob, True)
 
 
 @_advance_op.register_fake
-def _(k, v, k_caches, v_caches, k_scales, v_scales, rings, parents, tokens, target, pos, row_map, pos_out):
+def _(k, v, k_caches, v_caches, k_scales, v_scales, rings, parents, tokens, target, pos, row_map, pos_out, oob):
     B, T = tokens.shape
     return (pos.new_empty((B, T), dtype=torch.int32), pos.new_empty((B,), dtype=torch.int32), pos.new_empty((B, T), dtype=torch.int64))
 
@@ -108,20 +109,20 @@ def tree_advance(k, v, k_caches, v_caches, k_scales, v_scales, rings, parents: T
             return got
     if pos_out is pos:      # (an operator may not be told of one tensor as read and as written)
         new = torch.empty_like(pos)
-        got = _advance_op(k, v, k_caches, v_caches, k_scales, v_scales, rings, parents, tokens, target, pos, row_map, new)
+        got = _advance_op(k, v, k_caches, v_caches, k_scales, v_scales, rings, parents, tokens, target, pos, row_map, new, oob)
         pos.copy_(new)
         return got
-    return _advance_op(k, v, k_caches, v_caches, k_scales, v_scales, rings, parents, tokens, target, pos, row_map, pos_out)
+    return _advance_op(k, v, k_caches, v_caches, k_scales, v_scales, rings, parents, tokens, target, pos, row_map, pos_out, oob)
 
 
-@torch.library.custom_op("uvb200::kv_fork", mutates_args=("k_caches", "v_caches", "k_scales", "v_scales", "pos", "starts"))
+@torch.library.custom_op("uvb200::kv_fork", mutates_args=("k_caches", "v_caches", "k_scales", "v_scales", "pos", "starts", "oob"))
 def _fork_op(k_caches: Sequence[Tensor], v_caches: Sequence[Tensor], k_scales: Sequence[Tensor], v_scales: Sequence[Tensor],
-             rings: Sequence[bool], src: Tensor, dst: Tensor, pos: Tensor, starts: Tensor) -> None:
-    _lib.host().kv_fork(k_caches, v_caches, k_scales, v_scales, list(rings), src, dst, pos, starts, None, True)
+             rings: Sequence[bool], src: Tensor, dst: Tensor, pos: Tensor, starts: Tensor, oob: Optional[Tensor]) -> None:
+    _lib.host().kv_fork(k_caches, v_caches, k_scales, v_scales, list(rings), src, dst, pos, starts, oob, True)
 
 
 @_fork_op.register_fake
-def _(k_caches, v_caches, k_scales, v_scales, rings, src, dst, pos, starts):
+def _(k_caches, v_caches, k_scales, v_scales, rings, src, dst, pos, starts, oob):
     return None
 
 
@@ -133,4 +134,4 @@ def kv_fork(k_caches, v_caches, k_scales, v_scales, rings, src: Tensor, dst: Ten
     if not torch.compiler.is_compiling() and _lib.host().kv_fork(k_caches, v_caches, k_scales, v_scales, rings, src, dst, pos, starts,
                                                                  oob, False):
         return
-    _fork_op(k_caches, v_caches, k_scales, v_scales, rings, src, dst, pos, starts)
+    _fork_op(k_caches, v_caches, k_scales, v_scales, rings, src, dst, pos, starts, oob)
