@@ -102,3 +102,20 @@ def test_watched_calls_count_what_they_skip():
             got = call(watched)
             call(None)
         assert torch.equal(got, want) and int(plain) == int(watched) == skipped
+
+
+def test_indexes_of_any_integer_type():
+    from ultraviolet_b200.kernels import adjust_logits, tree_positions
+    x = torch.randn((2, 100), generator=_gen(1), device="cuda")
+    ids, bias = torch.tensor([3, 90, 3, 99], device="cuda"), torch.tensor([1.0, -2.0, 5.0, 0.5], device="cuda")
+    want = adjust_logits(x, bias_ids=ids.int(), bias=bias)
+    assert not torch.equal(want, adjust_logits(x))
+    for dtype in (torch.int64, torch.int16, torch.int8, torch.uint8):
+        assert torch.equal(adjust_logits(x, bias_ids=ids.to(dtype), bias=bias), want), dtype
+    far = torch.tensor([3, 90, 3, 2 ** 40], device="cuda")
+    assert torch.equal(adjust_logits(x, bias_ids=far, bias=bias)[:, :99], want[:, :99])
+    par, pos = torch.tensor([-1, 0, 1, 0, -2], device="cuda"), torch.tensor([10, 20], device="cuda")
+    for dtype in (torch.int64, torch.int32, torch.int16, torch.int8):
+        assert tree_positions(par.to(dtype), pos.to(torch.int16)).tolist() == [[10, 11, 12, 11, 10], [20, 21, 22, 21, 20]], dtype
+    # unsigned parents name no root: every node is absent
+    assert tree_positions(torch.tensor([0, 0, 255], dtype=torch.uint8, device="cuda"), pos).tolist() == [[10] * 3, [20] * 3]

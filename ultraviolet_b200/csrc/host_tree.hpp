@@ -52,14 +52,19 @@ Tensor index_of(const Tensor& t, int64_t B, const char* name) {
   TORCH_CHECK_VALUE(at::isIntegralType(t.scalar_type(), false), name, " has to hold integers; got ", t.scalar_type());
   return t.scalar_type() == at::kLong && t.is_contiguous() ? t : t.to(at::kLong).contiguous();
 }
+// Integers of any type as int32, those beyond lo .. hi (which name nothing either) as the nearer of the two.
+Tensor int32_of(const Tensor& t, int64_t lo, int64_t hi) {
+  if (t.scalar_type() == at::kInt) return t;
+  // (narrower types may not hold the bounds, and fit as they are)
+  return t.element_size() < 4 ? t.to(at::kInt) : t.to(at::kLong).clamp(lo, hi).to(at::kInt);
+}
 // parents (B, T) or (T,) as int32 with unit stride along T
 Tensor parents_of(const Tensor& p, int64_t B, int64_t T, int64_t& stride) {
   TORCH_CHECK_VALUE((p.dim() == 2 && p.size(0) == B && p.size(1) == T) || (p.dim() == 1 && p.size(0) == T), "parents have to be (", B, ", ", T,
                     ") or (", T, ",); got ", p.sizes());
   TORCH_CHECK_VALUE(at::isIntegralType(p.scalar_type(), false), "parents have to be integers; got ", p.scalar_type());
   TORCH_CHECK_VALUE(T <= 64, "a tree has at most 64 nodes; got ", T);
-  // (a parent that does not fit 32 bits must stay one that names no node)
-  Tensor q = p.scalar_type() == at::kInt ? p : p.clamp(-2, 64).to(at::kInt);
+  Tensor q = int32_of(p, -2, 64);
   if (T > 1 && q.stride(-1) != 1) q = q.contiguous();
   stride = q.dim() == 2 ? q.stride(0) : 0;
   return q;
@@ -358,7 +363,7 @@ std::optional<Tensor> adjust_logits(py::handle hx, const std::optional<std::tupl
     TORCH_CHECK_VALUE(ids_.sizes() == bias_.sizes() && (ids_.dim() == 1 || (ids_.dim() == 2 && ids_.size(0) == B)),
                       "bias_ids and bias have to be (", B, ", n) or (n,); got ", ids_.sizes(), " and ", bias_.sizes());
     TORCH_CHECK_VALUE(at::isIntegralType(ids_.scalar_type(), false) && bias_.scalar_type() == at::kFloat, "bias_ids have to be integers, bias float32");
-    ids = (ids_.scalar_type() == at::kInt ? ids_ : ids_.clamp(-1, INT32_MAX).to(at::kInt)).contiguous(), bias = bias_.contiguous();
+    ids = int32_of(ids_, -1, INT32_MAX).contiguous(), bias = bias_.contiguous();
     a.bias_ids = ids.const_data_ptr<int32_t>(), a.bias = bias.const_data_ptr<float>(), a.n_bias = (int)ids.size(-1);
     a.bias_stride = ids.dim() == 1 ? 0 : ids.size(-1);
   }
