@@ -119,3 +119,34 @@ def test_indexes_of_any_integer_type():
         assert tree_positions(par.to(dtype), pos.to(torch.int16)).tolist() == [[10, 11, 12, 11, 10], [20, 21, 22, 21, 20]], dtype
     # unsigned parents name no root: every node is absent
     assert tree_positions(torch.tensor([0, 0, 255], dtype=torch.uint8, device="cuda"), pos).tolist() == [[10] * 3, [20] * 3]
+
+
+@pytest.mark.parametrize("T", [1, 4])
+@pytest.mark.parametrize("B", [1, 2])
+def test_rows_of_an_odd_pitch(B, T):
+    """Slices of buffers whose rows are no multiple of 16 bytes: where one row or node is left of them, its dimension still has that stride."""
+    from ultraviolet_b200.kernels import kv_fork, tree_advance, tree_attention
+    S = 24
+    x = torch.randn((B, T, 10, 64), generator=_gen(T), device="cuda").to(torch.bfloat16)
+    kc, vc, ks, vs = _state(B, 1, S, 64, torch.bfloat16, 3)
+    rows = torch.zeros((3, T * 640 + 3), dtype=torch.bfloat16, device="cuda")[:, :T * 640].unflatten(1, (T, 10, 64))[:B]
+    nodes = torch.zeros((T + 1, 3, 645), dtype=torch.bfloat16, device="cuda")[..., :640].unflatten(2, (10, 64))[:T, :B].transpose(0, 1)
+    assert rows.stride(0) % 8 and nodes.stride(1) % 8
+    par, pos, zero = torch.arange(-1, T - 1, device="cuda"), torch.full((B,), 9, device="cuda"), torch.zeros(B, dtype=torch.long, device="cuda")
+    tok = torch.zeros((B, T), dtype=torch.long, device="cuda")
+    # and caches of which the same holds
+    wide = [torch.zeros((3, S * 64 + e), dtype=torch.int8, device="cuda")[:, :S * 64].unflatten(1, (1, S, 64))[:B] for e in (5, 9)]
+    wide[0].copy_(kc), wide[1].copy_(vc)
+    caches = [(kc, vc)] + ([tuple(wide)] if B == 1 else [])       # (rows of a cache that follow each other have to be aligned)
+    outs, ends = [], []
+    for src in (x, rows.copy_(x), nodes.copy_(x)):
+        for k, v in caches:
+            outs.append(tree_attention(src[:, :, :8], src[:, :, 8:9], src[:, :, 9:], k, v, pos, zero, par, 0.2, k_scale=ks, v_scale=vs))
+    for src in (x, rows, nodes):
+        for k, v in caches:
+            k[:, :, 9:9 + T], v[:, :, 9:9 + T] = 0, 0
+            tree_advance([src[:, :, 8:9]], [src[:, :, 9:]], [k], [v], [ks], [vs], [False], par, tok, tok, pos.clone())
+            ends.append((k.clone(), v.clone()))
+            kv_fork([k], [v], [ks], [vs], [False], zero[:1], zero[:1], pos, zero)
+    assert all(torch.equal(o, outs[0]) for o in outs)
+    assert all(torch.equal(a, b) for e in ends for a, b in zip(e, ends[0])) and ends[0][0][:, :, 9:9 + T].abs().sum() > 0

@@ -75,6 +75,8 @@ bool has_vectors(const Tensor& t) {
   for (int64_t i = 0; ok && i + 1 < t.dim(); ++i) ok = t.size(i) == 1 || t.stride(i) % 8 == 0;
   return ok;
 }
+// stride of a dimension; of one element, whose stride counts for nothing, none where it would not be a multiple of what kernels ask for
+int64_t step_of(const Tensor& t, int64_t i, int64_t multiple = 8) { return t.size(i) == 1 && t.stride(i) % multiple ? 0 : t.stride(i); }
 Tensor vectors_of(const Tensor& t) { return has_vectors(t) ? t : t.clone(at::MemoryFormat::Contiguous); }
 
 struct Cache {
@@ -154,16 +156,17 @@ std::optional<Tensor> tree_attention(py::handle hq, py::handle hk, py::handle hv
   q = vectors_of(q), k = vectors_of(k), v = vectors_of(v);
   uv_tree_attn_args a{};
   a.q = ro(q), a.k = ro(k), a.v = ro(v), a.dtype = code_of(q.scalar_type());
-  a.sqb = q.stride(0), a.sqt = q.stride(1), a.sqh = q.stride(2);
-  a.snkb = k.stride(0), a.snkt = k.stride(1), a.snkh = k.stride(2), a.snvb = v.stride(0), a.snvt = v.stride(1), a.snvh = v.stride(2);
+  a.sqb = step_of(q, 0), a.sqt = step_of(q, 1), a.sqh = step_of(q, 2);
+  a.snkb = step_of(k, 0), a.snkt = step_of(k, 1), a.snkh = step_of(k, 2), a.snvb = step_of(v, 0), a.snvt = step_of(v, 1), a.snvh = step_of(v, 2);
   a.parents = parents.const_data_ptr<int32_t>(), a.parents_stride = pstride;
   a.k_cache = kc.const_data_ptr<int8_t>(), a.v_cache = vc.const_data_ptr<int8_t>();
-  a.skb = kc.stride(0), a.skh = kc.stride(1), a.sks = kc.stride(2), a.svb = vc.stride(0), a.svh = vc.stride(1), a.svs = vc.stride(2);
+  a.skb = step_of(kc, 0, 16), a.skh = step_of(kc, 1, 16), a.sks = step_of(kc, 2, 16);
+  a.svb = step_of(vc, 0, 16), a.svh = step_of(vc, 1, 16), a.svs = step_of(vc, 2, 16);
   a.k_scale = static_cast<const uint16_t*>(ro(ks)), a.v_scale = static_cast<const uint16_t*>(ro(vs));
-  a.ssb = ks.stride(0), a.ssh = ks.stride(1), a.stb = vs.stride(0), a.sth = vs.stride(1);
+  a.ssb = step_of(ks, 0), a.ssh = step_of(ks, 1), a.stb = step_of(vs, 0), a.sth = step_of(vs, 1);
   a.pos = pos.const_data_ptr<int64_t>(), a.starts = starts.const_data_ptr<int64_t>();
   a.row_map = rm.defined() ? rm.const_data_ptr<int64_t>() : nullptr, a.n_rows = (int)y.rows;
-  a.out = out.mutable_data_ptr(), a.sob = out.stride(0), a.sot = out.stride(1), a.soh = out.stride(2);
+  a.out = out.mutable_data_ptr(), a.sob = step_of(out, 0), a.sot = step_of(out, 1), a.soh = step_of(out, 2);
   a.B = (int)B, a.T = (int)T, a.H = (int)H, a.KH = (int)y.KH, a.hd = (int)hd, a.S = (int)y.S;
   a.S_alloc = (int)row_alloc(kc, vc, ks, vs, y.S), a.window = (int)std::min<int64_t>(window, INT32_MAX);
   a.ring = ring < 0 ? window > 0 : ring != 0, a.scale = (float)scale, a.num_splits = (int)std::min<int64_t>(splits, INT32_MAX);
@@ -269,7 +272,8 @@ std::optional<std::tuple<Tensor, Tensor, Tensor>> tree_advance(const py::sequenc
   Tensor path = at::empty({B, T}, parents.options()), count = at::empty({B}, parents.options()), drawn = at::empty({B, T}, pos.options());
   uv_tree_advance_args a{};
   a.dtype = code_of(k0->scalar_type()), a.B = (int)B, a.T = (int)T, a.KH = (int)y.KH, a.hd = (int)y.hd, a.n_layers = (int)n;
-  a.skb = k0->stride(0), a.skt = k0->stride(1), a.skh = k0->stride(2), a.svb = v0->stride(0), a.svt = v0->stride(1), a.svh = v0->stride(2);
+  a.skb = step_of(*k0, 0), a.skt = step_of(*k0, 1), a.skh = step_of(*k0, 2);
+  a.svb = step_of(*v0, 0), a.svt = step_of(*v0, 1), a.svh = step_of(*v0, 2);
   a.parents = parents.const_data_ptr<int32_t>(), a.parents_stride = pstride;
   a.tokens = tokens.const_data_ptr<int64_t>(), a.target = target.const_data_ptr<int64_t>(), a.pos = pos.const_data_ptr<int64_t>();
   a.row_map = rm.defined() ? rm.const_data_ptr<int64_t>() : nullptr, a.n_rows = (int)y.rows;
