@@ -150,3 +150,26 @@ def test_rows_of_an_odd_pitch(B, T):
             kv_fork([k], [v], [ks], [vs], [False], zero[:1], zero[:1], pos, zero)
     assert all(torch.equal(o, outs[0]) for o in outs)
     assert all(torch.equal(a, b) for e in ends for a, b in zip(e, ends[0])) and ends[0][0][:, :, 9:9 + T].abs().sum() > 0
+
+
+def test_watched_logits_refuse_the_same_outputs():
+    from torch.utils._python_dispatch import TorchDispatchMode
+    from ultraviolet_b200.kernels import adjust_logits
+
+    class Watch(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+
+    x = torch.randn((2, 40), generator=_gen(1), device="cuda")
+    wrong = [torch.zeros(s, dtype=d, device="cuda") for s, d in (((3, 2, 40), torch.float32), ((1, 2, 40), torch.float32), ((2, 40), torch.int32),
+                                                                ((2, 40), torch.float64), ((2, 41), torch.float32))]
+    right = torch.zeros((2, 40), dtype=torch.float16, device="cuda")
+    for out in wrong:
+        with pytest.raises(ValueError):
+            adjust_logits(x, out=out)
+        with Watch(), pytest.raises(ValueError):
+            adjust_logits(x, out=out)
+        assert (out == 0).all()
+    with Watch():
+        assert adjust_logits(x, out=right) is right
+    assert torch.equal(right, x.half())

@@ -47,5 +47,7 @@ def adjust_logits(x: Tensor, *, softcap=None, history: Tensor | None = None, len
                                         False)
         if got is not None:
             return got
+    if out is not None and (out.shape != x.shape or out.dtype not in (torch.float32, torch.float16, torch.bfloat16)):
+        raise ValueError(f"out has to be float32, float16 or bfloat16 and like x; got {tuple(out.shape)} {out.dtype}")
     got = _adjust_op(x, cap, history, lengths, prompt_lengths, parents, tokens, *per_row, bias_ids, bias, allowed)
     return got if out is None else out.copy_(got)
