@@ -179,7 +179,7 @@ static int adjust_types(const uv_adjust_args& a, cudaStream_t st) {
   const bool vec = groups_meet<TI, TO>(a);
   // runs of 4096 entries where they fill the device twice, so that fewer blocks read the text; 1024 where there are few rows.  One row of
   // 16384: 6.1 us in runs of 4096, 4.3 of 1024; 63 rows of 50257 (819 runs of 4096) 10.5 and 13.3; 512 rows of 16384 26.4 and 33.6
-  if ((int64_t)a.B * a.T * ((a.V + 4095) / 4096) >= 2 * 148) launch_adjust<TI, TO, 256, 4>(a, vec, st);
+  if ((int64_t)a.B * a.T * ((a.V + 4095) / 4096) >= 2 * sm_count()) launch_adjust<TI, TO, 256, 4>(a, vec, st);
   else launch_adjust<TI, TO, 128, 2>(a, vec, st);
   return check_launch();
 }

@@ -7,6 +7,13 @@ namespace uv {
 
 constexpr int TREE_MAX = 64;
 
+// multiprocessors of the current device, as the rules for grids and parts count them
+inline int sm_count() {
+  int dev = 0, n = 148;
+  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+  return n;
+}
+
 // The cache's code of an fp16 or bf16 element: clamp(rint(x / s), -127, 127) with the IEEE quotient and ties to even, s an fp16 value or
 // 1e-30, inv within 2^-21 of 1 / s.  Without the division: x and s have at most 11 significant bits, so a quotient between 1/2 and
 // 127 that is not halfway between two codes is at least 2^-13 away from it, more than x * inv is off; and halfway is where the

@@ -600,12 +600,6 @@ static int default_parts(const uv_tree_attn_args& a, int row_tiles, int n_sm) {
   return s >= 2 && tiles >= (size == 0 ? 8 : 12) ? 2 : 1;
 }
 
-static int sm_count() {
-  int dev = 0, n = 148;
-  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
-  return n;
-}
-
 struct TreePlan {
   int R, splits;
   bool cluster;

@@ -915,11 +915,7 @@ __global__ void __launch_bounds__(256) tree_tc_merge_kernel(const __grid_constan
 }
 
 // ------------------------------------------------------------------------------------------------ host side
-static int tc_ctas(int hd) {
-  int dev = 0, n = 148;
-  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
-  return (hd > 64 ? 1 : 2) * n;
-}
+static int tc_ctas(int hd) { return (hd > 64 ? 1 : 2) * sm_count(); }
 static int64_t tc_units(const uv_tree_attn_args& a) {
   return (int64_t)a.B * a.KH * ((a.T * (a.H / a.KH) + TT_ROWS - 1) / TT_ROWS);
 }
