@@ -173,3 +173,43 @@ def test_watched_logits_refuse_the_same_outputs():
     with Watch():
         assert adjust_logits(x, out=right) is right
     assert torch.equal(right, x.half())
+
+
+def _exact(q, k, v, kc, vc, ks, vs, pos, parents, scale):
+    """One row in 64 bits, starts 0: the mean of the values and of their magnitudes, (T, H, hd) each."""
+    from oracle import kv as okv
+    T, H, hd = q.shape
+    keys, vals = [], []
+    for x, c, s, to in ((k, kc, ks, keys), (v, vc, vs, vals)):
+        codes, scales = (torch.from_numpy(a).to(q.device).double() for a in okv.quantize_kv(x.float().cpu().numpy()))     # (T, K, hd), (T, K)
+        to += [torch.cat([c[:, :pos].double() * s[:, :pos, None].double(), (codes * scales[..., None]).transpose(0, 1)], 1)]
+    keys, vals = keys[0], vals[0]                                                           # (K, pos + T, hd)
+    G = H // keys.size(0)
+    up = [ot.path_up(parents, t) for t in range(T)]
+    s = torch.einsum("tkgd,knd->ktgn", q.double().view(T, -1, G, hd), keys) * scale
+    for t in range(T):
+        hidden = torch.ones(T, dtype=torch.bool, device=q.device)
+        hidden[up[t]] = False
+        s[:, t, :, pos:].masked_fill_(hidden, float("-inf"))
+    w = torch.softmax(s, -1)
+    there = torch.tensor([len(u) > 0 for u in up], device=q.device)[:, None, None]
+    mean = lambda x: torch.einsum("ktgn,knd->tkgd", w, x).reshape(T, H, hd) * there
+    return mean(vals), mean(vals.abs())
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("route", sorted(ROUTES))
+def test_attention_within_what_its_roundings_leave(route, dtype):
+    """Half an ulp of the output; a weight times its value's scale is rounded to 11 bits, so that the mean moves by up to 2**-11 of
+    A = sum w |V| / sum w, and scores of 32 .. 128 exact products summed in 32 bits move it by less than as much again; what is
+    rounded below fp16's smallest normal is off by at most 2**-25 of the largest contribution a key, all of it below N 2**-25 max A."""
+    B, T, H, K, hd, S, splits = ROUTES[route]
+    run, x, ks, vs, pos, par = _call(route, dtype, "padded")
+    got = run(x)
+    kc, vc = _state(B, K, S, hd, dtype, T)[:2]
+    for b in (0, B - 1):
+        q, k, v = x[b].split([H, K, K], 1)
+        ref, size = _exact(q, k, v, kc[b], vc[b], ks[b], vs[b], int(pos[b]), par[b].tolist(), 0.14)
+        bound = 1.01 * UNIT[dtype] * 2 * ref.abs() + 2.0 ** -10 * size + S * 2.0 ** -25 * size.max() + 1e-7
+        err = (got[b].double() - ref).abs()
+        assert (err <= bound).all(), float((err / bound).max())
