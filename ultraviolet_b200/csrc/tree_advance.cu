@@ -54,10 +54,10 @@ __device__ __forceinline__ int tree_walk(const int32_t* parents, const int64_t* 
 }
 
 // A block per tree.  Every warp walks the tree for itself (a few ballots), then a group of HD / 8 lanes takes a vector, 8 elements a
-// lane: the accepted nodes' keys and values of all layers are far apart in memory and few, so what bounds it is the latency of the chain
-// pos, parents, tokens -> vectors -> codes, and two vectors a group are in flight.
-// Measured on a B200: 2.9 us for one tree of 4 nodes in 10 layers, 11.8 us for 256 trees of 16 nodes (two blocks on most SMs, a quarter of
-// the issue slots used).  Four blocks to a tree took 12.7 us, a layer to each of 16 warps 12.4 (and 4.8 for the one tree).
+// lane: the accepted nodes' keys and values of all layers are far apart in memory and few, so what bounds it is latency: the chain pos,
+// parents, tokens -> vectors -> codes, and, with two vectors a group in flight, a round of loads for every 64 vectors of 64 elements.
+// Measured on a B200: 3.1 us for one tree of 4 nodes in 10 layers, 11.7 us for 256 trees of 16 nodes, whose paths of nine make 180 vectors
+// (three rounds; two blocks on most SMs, a quarter of the issue slots used).  Four blocks to a tree took 12.7 us, a layer to each of 16 warps 12.4 (and 4.8 for the one tree).
 template <typename T, int HD>
 __global__ void __launch_bounds__(ADV_WARPS * 32) tree_advance_kernel(const __grid_constant__ AdvanceParams P) {
   constexpr int LV = HD / 8, GROUPS = ADV_WARPS * 32 / LV;

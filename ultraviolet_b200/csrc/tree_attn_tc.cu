@@ -25,7 +25,8 @@
 // slots), 2590 of 64 rows (0.58 us, 61 %); the softmax's own arithmetic is 1640 of them, conversion some 900, the rest barriers and
 // bookkeeping.  Around the tiles 12 us (ranges, queries, the first conversion, the epilogue), with units in pieces 30.  Measured, 8 heads of
 // 64 over one kv head: 64 rows of 16 nodes over 8192 positions 72 us (0.99 TB/s, 239 TFLOP/s), 256 rows of 8 nodes over 64 .. 2304 positions
-// 53 (the longest row's 37 tiles); 2 x 128 under 4 heads each, 3 rows of 61 nodes over 20001 .. 60007 positions 86 (349 TFLOP/s).
+// 53 (the longest row's 37 tiles); 2 x 128 under 4 heads each, 3 rows of 61 nodes over 20001 .. 60007 positions 87 (347 TFLOP/s):
+// 244 query rows of a kv head are two units, each of which copies and converts the same keys and values for itself.
 //
 // What does not run for every tile is kept small (rolled loops, functions out of line): a CTA runs most of it once, and then a
 // line of instructions costs its fetch, not its execution.
@@ -928,7 +929,7 @@ static int tc_grid(const uv_tree_attn_args& a, bool split) {
   const int64_t most = split ? tc_most_tiles(a) / 2 + 1 : tc_units(a), fit = tc_ctas(a.hd);
   return (int)(most < fit ? most : fit);
 }
-// Whole units or runs of tiles.  Whole: as long as the longest unit takes, 12 us and 1.25 a tile with one CTA on a multiprocessor, 1.45 with
+// Whole units or runs of tiles, by the cache's length (the rows' own are on the device).  Whole: as long as the longest unit takes, 12 us and 1.25 a tile with one CTA on a multiprocessor, 1.45 with
 // two; with two tiles at a time 12 us and 0.78, or 17 us and 1.16.  Runs: 30 us -- partials and the merging launch -- and 0.71 us (two tiles
 // at a time 0.55; 0.8 for head_dim 128) a tile of a multiprocessor, whatever the rows' lengths are.  (Measured at 64 to 296 rows of 60 to
 // 32768 positions; 120 rows of 8 nodes over 2304: whole 41 us, runs 51.)
