@@ -88,3 +88,19 @@ def test_tree_steps_are_the_same_with_dependent_launches():
         assert got.returncode == 0, got.stderr[-2000:]
         out.append(got.stdout.split()[-1])
     assert out[0] == out[1]
+
+
+def test_tree_kernels_that_give_up_wait_for_what_is_under_way():
+    """A kernel whose wait has run out ends behind its own copies and products, by another bounded wait: what arrives later would land in
+    the shared memory, or the tensor memory, of whoever has it then."""
+    kernels = _kernels()
+    rows, tc = kernels["tree_rows_kernel"], kernels["tree_tc_kernel"]
+    after = rows[rows.index("lost = s_dead"):]
+    assert re.search(r"if \(lost && producer.*?tc_mbar_wait\(tc_smem_u32\(&full\[", after, re.S) and "issued" in after
+    end = tc[tc.rindex("__syncthreads()"):]
+    commit, wait, free = (end.index(x) for x in ("tc_commit(tc_smem_u32(&sh.drained))", "tc_mbar_wait(tc_smem_u32(&sh.drained)", "tcgen05.dealloc"))
+    assert commit < wait < free
+    with open(os.path.join(CSRC, "tree_attn_tc.cu")) as f:      # the codes come by cp.async, which each thread waits for
+        body = f.read()
+    convert = body[body.index("void convert_tiles"):body.index("void mask_scores")]
+    assert convert.rstrip().rindex("cp.async.wait_all") > convert.rindex("mbar_arrive_one")

@@ -173,9 +173,10 @@ __global__ void __launch_bounds__(TR_THREADS) tree_rows_kernel(const __grid_cons
   };
 
   bool dead = false;
+  int issued = min(ntile, TR_STAGES);       // tiles asked for (the producer's count)
   if constexpr (BULK) {
     if (producer && lane == 0)
-      for (int j = 0; j < ntile && j < TR_STAGES; ++j) issue(t0 + j, j);
+      for (int j = 0; j < issued; ++j) issue(t0 + j, j);
   } else if (ntile > 0) {
     load_pieces(t0, 0);
   }
@@ -411,13 +412,13 @@ __global__ void __launch_bounds__(TR_THREADS) tree_rows_kernel(const __grid_cons
   if constexpr (BULK) {
     if (producer) {
       if (lane == 0)
-        for (int j = TR_STAGES; j < ntile; ++j) {
-          const int s = j % TR_STAGES;
-          if (!tc_mbar_wait(tc_smem_u32(&empty[s]), (uint32_t)((j / TR_STAGES - 1) & 1))) {
+        for (; issued < ntile; ++issued) {
+          const int s = issued % TR_STAGES;
+          if (!tc_mbar_wait(tc_smem_u32(&empty[s]), (uint32_t)((issued / TR_STAGES - 1) & 1))) {
             dead = true;
             break;
           }
-          issue(t0 + j, s);
+          issue(t0 + issued, s);
         }
     } else {
       for (int it = 0; it < ntile; ++it) {
@@ -451,6 +452,10 @@ __global__ void __launch_bounds__(TR_THREADS) tree_rows_kernel(const __grid_cons
   // ---- merge: the warps' states through shared memory (over the ring: every copy has landed, unless the CTA gave one up: then its
   //      part is reported empty, and the status word says that the output is not to be used)
   const bool lost = s_dead != 0;
+  if constexpr (BULK)
+    if (lost && producer && lane == 0)        // the CTA does not end before its own copies, or their waits, have
+      for (int j = max(0, issued - TR_STAGES); j < issued; ++j)
+        tc_mbar_wait(tc_smem_u32(&full[j % TR_STAGES]), (uint32_t)((j / TR_STAGES) & 1));
   float* const mg_o = reinterpret_cast<float*>(smem);
   float* const mg_m = mg_o + TR_WARPS * ROWS * HD;
   float* const mg_l = mg_m + TR_WARPS * ROWS;

@@ -25,7 +25,7 @@
 // slots), 2590 of 64 rows (0.58 us, 61 %); the softmax's own arithmetic is 1640 of them, conversion some 900, the rest barriers and
 // bookkeeping.  Around the tiles 12 us (ranges, queries, the first conversion, the epilogue), with units in pieces 30.  Measured, 8 heads of
 // 64 over one kv head: 64 rows of 16 nodes over 8192 positions 72 us (0.99 TB/s, 239 TFLOP/s), 256 rows of 8 nodes over 64 .. 2304 positions
-// 53 (the longest row's 37 tiles); 2 x 128 under 4 heads each, 3 rows of 61 nodes over 20001 .. 60007 positions 87 (347 TFLOP/s):
+// 53 (the longest row's 37 tiles); 2 x 128 under 4 heads each, 3 rows of 61 nodes over 20001 .. 60007 positions 87 (346 TFLOP/s):
 // 244 query rows of a kv head are two units, each of which copies and converts the same keys and values for itself.
 //
 // What does not run for every tile is kept small (rolled loops, functions out of line): a CTA runs most of it once, and then a
@@ -107,6 +107,7 @@ struct TcRow {
 };
 struct TcShared {
   uint64_t kv_full[2][TT_NK], kv_empty[2][TT_NK], p_full[2], s_full[TT_NSC], o_done[2], piece_full, q_full;   // s_full: the products and both scales
+  uint64_t drained;                    // every product issued so far, where the CTA gives up
   int lv_max[TT_NSC];                  // floor(log2) of a tile's largest value scale
   uint32_t tmem;
   int dead;
@@ -871,6 +872,11 @@ __global__ void __launch_bounds__(TT_THREADS, TcSmem<HD>::CTAS) tree_tc_kernel(c
   __syncthreads();
   if (tid == 0 && sh.dead && a.status) atomicOr(a.status, 1);
   if (warp == 12) {
+    if (!likely(sh.dead == 0)) {                 // products may be under way: the CTA does not end before them, or this wait
+      if (elect_one()) tc_commit(tc_smem_u32(&sh.drained));
+      tc_mbar_wait(tc_smem_u32(&sh.drained), 0u);
+      __syncwarp();
+    }
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(M::COLS) : "memory");
   }
