@@ -95,8 +95,7 @@ def test_tree_kernels_that_give_up_wait_for_what_is_under_way():
     the shared memory, or the tensor memory, of whoever has it then."""
     kernels = _kernels()
     rows, tc = kernels["tree_rows_kernel"], kernels["tree_tc_kernel"]
-    after = rows[rows.index("lost = s_dead"):]
-    assert re.search(r"if \(lost && producer.*?tc_mbar_wait\(tc_smem_u32\(&full\[", after, re.S) and "issued" in after
+    assert re.search(r"if \(lost && producer && lane == 0\) drain_copies\(full, issued\)", rows[rows.index("lost = s_dead"):])
     end = tc[tc.rindex("__syncthreads()"):]
     commit, wait, free = (end.index(x) for x in ("tc_commit(tc_smem_u32(&sh.drained))", "tc_mbar_wait(tc_smem_u32(&sh.drained)", "tcgen05.dealloc"))
     assert commit < wait < free

@@ -80,6 +80,12 @@ template <int HD, int R> struct TreeSmem {
   static constexpr int BYTES = PART + ROWS * (HD + 2) * 4;
 };
 
+// Waits for the last copies asked for, after a wait that ran out (out of line: what is not run costs no instruction lines).
+__device__ __noinline__ void drain_copies(uint64_t* full, int issued) {
+  for (int j = max(0, issued - TR_STAGES); j < issued; ++j)
+    tc_mbar_wait(tc_smem_u32(&full[j % TR_STAGES]), (uint32_t)((j / TR_STAGES) & 1));
+}
+
 template <typename QT, int HD, int R, bool BULK>
 __global__ void __launch_bounds__(TR_THREADS) tree_rows_kernel(const __grid_constant__ TreeParams P) {
   using L = TreeStage<HD>;
@@ -173,10 +179,10 @@ __global__ void __launch_bounds__(TR_THREADS) tree_rows_kernel(const __grid_cons
   };
 
   bool dead = false;
-  int issued = min(ntile, TR_STAGES);       // tiles asked for (the producer's count)
+  int issued = ntile;                       // tiles asked for, once the producer is done
   if constexpr (BULK) {
     if (producer && lane == 0)
-      for (int j = 0; j < issued; ++j) issue(t0 + j, j);
+      for (int j = 0; j < ntile && j < TR_STAGES; ++j) issue(t0 + j, j);
   } else if (ntile > 0) {
     load_pieces(t0, 0);
   }
@@ -412,13 +418,13 @@ __global__ void __launch_bounds__(TR_THREADS) tree_rows_kernel(const __grid_cons
   if constexpr (BULK) {
     if (producer) {
       if (lane == 0)
-        for (; issued < ntile; ++issued) {
-          const int s = issued % TR_STAGES;
-          if (!tc_mbar_wait(tc_smem_u32(&empty[s]), (uint32_t)((issued / TR_STAGES - 1) & 1))) {
-            dead = true;
+        for (int j = TR_STAGES; j < ntile; ++j) {
+          const int s = j % TR_STAGES;
+          if (!tc_mbar_wait(tc_smem_u32(&empty[s]), (uint32_t)((j / TR_STAGES - 1) & 1))) {
+            dead = true, issued = j;
             break;
           }
-          issue(t0 + issued, s);
+          issue(t0 + j, s);
         }
     } else {
       for (int it = 0; it < ntile; ++it) {
@@ -453,9 +459,7 @@ __global__ void __launch_bounds__(TR_THREADS) tree_rows_kernel(const __grid_cons
   //      part is reported empty, and the status word says that the output is not to be used)
   const bool lost = s_dead != 0;
   if constexpr (BULK)
-    if (lost && producer && lane == 0)        // the CTA does not end before its own copies, or their waits, have
-      for (int j = max(0, issued - TR_STAGES); j < issued; ++j)
-        tc_mbar_wait(tc_smem_u32(&full[j % TR_STAGES]), (uint32_t)((j / TR_STAGES) & 1));
+    if (lost && producer && lane == 0) drain_copies(full, issued);       // the CTA does not end before its own copies
   float* const mg_o = reinterpret_cast<float*>(smem);
   float* const mg_m = mg_o + TR_WARPS * ROWS * HD;
   float* const mg_l = mg_m + TR_WARPS * ROWS;
