@@ -173,3 +173,16 @@ def test_the_hosts_positions_follow_a_run():
     run = _runner(m, [[1, 2, 3, 4], [4, 3, 2, 1]], 12, branches=1, depth=3, temperature=0.0)
     run.run()
     assert run.st.host_pos.tolist() == run.st.pos.tolist() and int(run.st.pos.min()) >= 3 + 12
+
+
+def test_a_first_step_that_is_refused_leaves_the_run_as_it_was():
+    m = _model("tiny")
+    run = _runner(m, [[1, 2, 3, 4], [4, 3, 2, 1]], 6, branches=1, depth=3, temperature=0.0, **_favour(m, 7))
+    run.adjust["allowed"] = torch.full((2, 1), -1, dtype=torch.int32, device=DEV)      # too few words for the vocabulary
+    parents = run.parents.clone()
+    with pytest.raises(ValueError):
+        run.step()
+    assert torch.equal(run.parents, parents) and run.steps_run == 0
+    run.adjust["allowed"] = None
+    run.run()
+    assert run.completions() == [[7] * 6] * 2

@@ -142,13 +142,15 @@ class TreeRunner:
         saved = [t.clone() for t in kept]
         s = torch.cuda.Stream(dev)
         s.wait_stream(torch.cuda.current_stream(dev))
-        with torch.cuda.stream(s):
-            # warm-up without a node in any tree: an accepted path would wrap over ring slots that the real first step still reads
-            self.parents.fill_(-2)
-            self._body()
+        try:
+            with torch.cuda.stream(s):
+                # warm-up without a node in any tree: an accepted path would wrap over ring slots that the real first step still reads
+                self.parents.fill_(-2)
+                self._body()
+        finally:
+            torch.cuda.current_stream(dev).wait_stream(s)
             for t, v in zip(kept, saved):
                 t.copy_(v)
-        torch.cuda.current_stream(dev).wait_stream(s)
         g = torch.cuda.CUDAGraph()
         with torch.cuda.graph(g, capture_error_mode="thread_local"):
             self._body()
